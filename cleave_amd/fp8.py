@@ -131,7 +131,9 @@ def _product_dims(shape, b: Fp8Tensor, trans_b: bool, what: str) -> tuple:
 
 
 def matmul_fp8(a: Fp8Tensor, b: Fp8Tensor, trans_b: bool = False, dtype: str = "f32", out=None):
-    """C = a b (b quantised with block_rows=128) or, with trans_b, a b^T, as f32 or bf16."""
+    """C = a b (b quantised with block_rows=128) or, with trans_b, a b^T, as f32 or bf16.
+    bf16 results of more than 32 rows keep products to 2^-13 of the largest of 8; f32
+    ones, and those of fewer rows, are f32 sums."""
     M, N, K = _product_dims(_held(a, "matmul_fp8").shape, _held(b, "matmul_fp8"), trans_b, "matmul_fp8")
     out = out if out is not None else ca.empty((M, N), _wide(dtype, "matmul_fp8"))
     call(f"cleave_hip_matmul_fp8_{_wide(out.dtype, 'matmul_fp8')}", *a.args, *b.args, out.ptr, out.size, M, N, K,
@@ -140,8 +142,8 @@ def matmul_fp8(a: Fp8Tensor, b: Fp8Tensor, trans_b: bool = False, dtype: str = "
 
 
 def linear_fp8(x, w: Fp8Tensor, trans_b: bool = False, dtype: str = "f32", out=None, x8: Fp8Tensor | None = None):
-    """y = Q(x) w (or Q(x) w^T), Q(x) being x quantised by rows; x8 receives Q(x),
-    which weight_grad_fp8 reads in the backward pass."""
+    """y = Q(x) w (or Q(x) w^T), Q(x) being x quantised by rows, summed as matmul_fp8 sums;
+    x8 receives Q(x), which weight_grad_fp8 reads in the backward pass."""
     M, N, K = _product_dims(_matrix(x, "linear_fp8"), _held(w, "linear_fp8"), trans_b, "linear_fp8")
     out = out if out is not None else ca.empty((M, N), _wide(dtype, "linear_fp8"))
     if x8 is not None:
