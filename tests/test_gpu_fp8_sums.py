@@ -7,7 +7,11 @@
                                             counts as 2^-6), at most 7 of them; sums rounded
                                             down, one f32 step (2^-23 of at most sum |a||b|)
                                             for each 8 and for each joined slice; the result is
-                                            the nearest bf16 to a value within that of a b"""
+                                            the nearest bf16 to a value within that of a b
+
+and, exactly, on small integers: with products up to 64 of at least 1 nothing is cut off and
+every partial sum is a whole number below 2^24, so each k, lane, tile and ragged edge has to
+be in its place once."""
 from __future__ import annotations
 
 import numpy as np
@@ -83,3 +87,56 @@ def test_bf16_sums_lose_no_more_than_stated(hip, M, N, K, trans_b):
         low, high = cut_off(tuple(p[r] for p in pa), tuple(p[:, c] for p in pb), K)
         some = got[np.ix_(r, c)]
         assert ((low <= some) & (some <= high)).all()
+
+
+INTEGERS = [(33, 70, 300), (100, 130, 129), (64, 64, 8192), (100, 200, 2100), (1000, 33, 2049),  # 64 x 64, whole and in slices
+            (1500, 1400, 700), (1409, 1537, 200),                                               # 128 x 128
+            (2817, 3001, 300), (2900, 2817, 8300),               # 256 x 256, a tile a workgroup; past 64 k-blocks
+            (4500, 4700, 300), (4353, 4097, 129), (4200, 4300, 8333),   # several tiles a workgroup, edges after whole ones
+            (8192, 8192, 256), (12288, 5632, 384)]               # ... and C of 128 MiB and more, in whole lines
+
+
+@pytest.mark.parametrize("M,N,K", INTEGERS)
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_bf16_results_of_integers_are_exact(hip, M, N, K, trans_b):
+    rng = rng_of("bf16 integers", M, N, K, trans_b)
+    a = rng.integers(-8, 9, (M, K)).astype(np.float32)
+    b = rng.integers(-8, 9, (K, N)).astype(np.float32)
+    a8 = hip.quantize_fp8(hip.from_numpy(a))
+    b8 = hip.quantize_fp8(hip.from_numpy(np.ascontiguousarray(b.T) if trans_b else b), 128)
+    first = hip.matmul_fp8(a8, b8, trans_b=trans_b, dtype="bf16").numpy()
+    assert np.array_equal(first, ref.to_bf16(a @ b))  # an f32 product of whole numbers below 2^24: exact in any order
+    assert np.array_equal(first, hip.matmul_fp8(a8, b8, trans_b=trans_b, dtype="bf16").numpy())
+
+
+@pytest.mark.parametrize("M,N,K", [(140, 260, 300), (1500, 1400, 130), (2900, 2817, 300), (4500, 4700, 200)])
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_bf16_nan_stays_in_its_row_and_column(hip, M, N, K, trans_b):
+    rng = rng_of("bf16 nan", M, N, K)
+    a = rng.standard_normal((M, K), np.float32)
+    b = rng.standard_normal((K, N), np.float32)
+    a[3, K - 1] = a[M - 1, 0] = np.nan
+    b[K - 1, N - 1] = b[0, 5] = np.nan
+    a8 = hip.quantize_fp8(hip.from_numpy(a))
+    b8 = hip.quantize_fp8(hip.from_numpy(np.ascontiguousarray(b.T) if trans_b else b), 128)
+    c = values(hip.matmul_fp8(a8, b8, trans_b=trans_b, dtype="bf16"))
+    want = np.zeros((M, N), bool)
+    want[[3, M - 1]] = True
+    want[:, [5, N - 1]] = True
+    assert np.array_equal(np.isnan(c), want)
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_several_tiles_a_workgroup_into_offset_memory(hip, trans_b):
+    # C on no 16-byte boundary and of whole 128-byte lines' length: its neighbours stay, and it is not streamed
+    M, N, K = 8192, 8192, 128
+    rng = rng_of("offset walk", trans_b)
+    a = rng.integers(-8, 9, (M, K)).astype(np.float32)
+    b = rng.integers(-8, 9, (K, N)).astype(np.float32)
+    a8 = hip.quantize_fp8(hip.from_numpy(a))
+    b8 = hip.quantize_fp8(hip.from_numpy(np.ascontiguousarray(b.T) if trans_b else b), 128)
+    raw = hip.from_numpy(np.full(M * N + 2, 0x40E0, np.uint16), "bf16")
+    hip.matmul_fp8(a8, b8, trans_b=trans_b, out=raw.sub(1, (M, N)))
+    got = raw.numpy()
+    assert got[0] == 0x40E0 and got[-1] == 0x40E0
+    assert np.array_equal(got[1:-1].reshape(M, N), ref.to_bf16(a @ b))
