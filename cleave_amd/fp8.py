@@ -80,13 +80,19 @@ def _held(t, what: str) -> "Fp8Tensor":
 
 
 def _room(out, shape, block_rows: int, what: str) -> "Fp8Tensor":
-    """out, if it can hold the result, or a new Fp8Tensor."""
+    """out, if it can hold the result, or a new Fp8Tensor.  What out is labelled as stays until it holds that."""
     if out is None:
         return empty_fp8(shape, block_rows)
     if tuple(_held(out, what).shape) != tuple(shape):
         raise ValueError(f"{what}: out holds {tuple(out.shape)}, the result is {tuple(shape)}")
-    out.block_rows = block_rows
     return out
+
+
+def _filled(t: "Fp8Tensor | None", block_rows: int = 1) -> "Fp8Tensor | None":
+    """t, now that the library has written it with that many rows to a scale."""
+    if t is not None:
+        t.block_rows = block_rows
+    return t
 
 
 def empty_fp8(shape, block_rows: int = 1) -> Fp8Tensor:
@@ -108,7 +114,7 @@ def quantize_fp8(x, block_rows: int = 1, out: Fp8Tensor | None = None) -> Fp8Ten
         raise ValueError(f"quantize_fp8: block_rows is 1 or {BLOCK}, not {block_rows}")
     out = _room(out, (rows, cols), block_rows, "quantize_fp8")
     call(f"cleave_hip_quantize_fp8_{sfx}", x.ptr, x.size, *out.args, rows, cols, block_rows)
-    return out
+    return _filled(out, block_rows)
 
 
 def dequantize_fp8(t: Fp8Tensor, dtype: str = "f32", out=None):
@@ -150,6 +156,7 @@ def linear_fp8(x, w: Fp8Tensor, trans_b: bool = False, dtype: str = "f32", out=N
         x8 = _room(x8, (M, K), 1, "linear_fp8")
     call(f"cleave_hip_linear_fp8_{_wide(x.dtype, 'linear_fp8')}_{_wide(out.dtype, 'linear_fp8')}", x.ptr, x.size,
          *w.args, out.ptr, out.size, *(x8.args if x8 is not None else _NONE), M, N, K, int(trans_b))
+    _filled(x8)
     return out
 
 
@@ -174,7 +181,7 @@ def _act(act: str, z, save: bool, h8: Fp8Tensor | None, z8: Fp8Tensor | None):
     if save or z8 is not None:
         z8 = _room(z8, shape, 1, what)
     call(f"cleave_hip_{act}_fp8_{sfx}", z.ptr, z.size, *h8.args, *(z8.args if z8 is not None else _NONE), *shape)
-    return h8, z8
+    return _filled(h8), _filled(z8)
 
 
 def relu_fp8(z, h8: Fp8Tensor | None = None) -> Fp8Tensor:
@@ -204,7 +211,7 @@ def _act_bwd(act: str, z8: Fp8Tensor, g, out, out8: Fp8Tensor | None, codes: boo
         out8 = _room(out8, shape, 1, what)
     call(f"cleave_hip_{act}_bwd_fp8_{sfx}", *z8.args, g.ptr, g.size, out.ptr, out.size,
          *(out8.args if out8 is not None else _NONE), *shape)
-    return out, out8
+    return out, _filled(out8)
 
 
 def relu_bwd_fp8(h8: Fp8Tensor, g, out=None, out8: Fp8Tensor | None = None, codes: bool = True):
