@@ -5,7 +5,7 @@
 // One pass each: a row's block of 128 lies in 16 lanes of 8 values, so its
 // largest magnitude is four DPP steps, and the values are still in registers
 // when the scale is known.  All of it is bound by HBM bytes: bf16 65536 x 4096
-// sigmoid with its checkpoint 193 us (1.08 GB, 5.6 TB/s), its backward with both
+// sigmoid with its checkpoint 187 us (1.08 GB, 5.8 TB/s), its backward with both
 // results 276 us (1.62 GB, 5.9 TB/s), an f32 8192^2 weight 57 us (0.34 GB, 5.9
 // TB/s); 1000 x 500 is one launch, 3 us of it the kernel.
 #include <type_traits>
@@ -121,8 +121,11 @@ __device__ __forceinline__ uint2 keep_positive(uint2 q, const float (&h)[8]) {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// fwd_near: act(z) where no |z| is past kNear; fwd: any z, and the same bits for those.
+// So which of them a wave takes changes nothing, and a row's codes do not depend on
+// its neighbours.
 struct Relu {
-    static constexpr float kClip = __builtin_inff();
+    static constexpr float kClip = __builtin_inff(), kNear = kClip;
     static __device__ __forceinline__ float fwd_near(float z) { return fwd(z); }
     static __device__ __forceinline__ float fwd(float z) { return z > 0.0f ? z : (z != z ? z : 0.0f); }
     // g where z > 0, whatever g holds elsewhere
@@ -134,19 +137,16 @@ __device__ __forceinline__ float exp2_down(float t) {
     const float e = __builtin_amdgcn_exp2f(low ? t + 64.0f : t);
     return low ? e * 0x1.0p-64f : e;
 }
-// Everything is written in u = e^-|z| (e^-2|z|), which neither overflows nor
-// cancels for a large |z|.
 struct Sigmoid {
-    static constexpr float kClip = 32.0f;
-    // where every |z| is at most kClip
+    // past kNear, e^-z or its reciprocal leaves the normal floats; there 1 + e^-z is e^-z
+    static constexpr float kClip = 32.0f, kNear = 87.0f;
     static __device__ __forceinline__ float fwd_near(float z) {
         return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
     }
     static __device__ __forceinline__ float fwd(float z) {
-        const float u = exp2_down(-kLog2e * __builtin_fabsf(z));
-        const float r = __builtin_amdgcn_rcpf(1.0f + u);
-        return z < 0.0f ? u * r : r;
+        return z < -kNear ? exp2_down(kLog2e * z) : fwd_near(z);
     }
+    // in u = e^-|z|, which neither overflows nor cancels for a large |z|
     static __device__ __forceinline__ float bwd(float z, float g) {
         const float u = __builtin_amdgcn_exp2f(-kLog2e * __builtin_fabsf(z));
         const float r = __builtin_amdgcn_rcpf(1.0f + u);
@@ -154,9 +154,9 @@ struct Sigmoid {
     }
 };
 struct Tanh {
-    static constexpr float kClip = 16.0f;
+    static constexpr float kClip = 16.0f, kNear = __builtin_inff();
     static __device__ __forceinline__ float fwd_near(float z) { return fwd(z); }
-    static __device__ __forceinline__ float fwd(float z) {
+    static __device__ __forceinline__ float fwd(float z) {  // in u = e^-2|z|
         const float a = __builtin_fabsf(z), u = __builtin_amdgcn_exp2f(-2.0f * kLog2e * a);
         const float far = (1.0f - u) * __builtin_amdgcn_rcpf(1.0f + u), w = z * z;
         // 1 - u loses the small ones: the series to z^7, 2e-9 off at 1/8
@@ -315,10 +315,9 @@ __global__ __launch_bounds__(kThreads) void act_kernel(const T* __restrict__ z, 
     for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int kb) {
         const int n = row < rows ? cols - c : 0;
         float h[8];
-        // The plain way for blocks whose every |z| is at most kClip, which need no
-        // clipping either; a NaN or an infinity takes the other.
-        const bool near = !__any(!(amax8(v[i]) <= Act::kClip));
-        if (near) {
+        // One way for the whole wave; an infinity (or a signalling NaN) is past any bound.
+        const float top = amax8(v[i]);
+        if (Act::kNear == __builtin_inff() || !__any(!(top <= Act::kNear))) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] = Act::fwd_near(v[i][e]);
         } else {
@@ -335,7 +334,7 @@ __global__ __launch_bounds__(kThreads) void act_kernel(const T* __restrict__ z, 
         if (row < rows) *reinterpret_cast<uint2*>(hq + row * pitch + c) = w;
         if ((threadIdx.x & 15) == 0) hs[kb * sp + row] = (uint8_t)sb;
         if constexpr (KEEP) {
-            if (!near) {
+            if (__any(!(top <= Act::kClip))) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[i][e] = clip(v[i][e], Act::kClip);
             }

@@ -168,3 +168,41 @@ def test_derivative_scales_and_padding(hip, rows, cols, dtype, act):
     dz, dz8 = {"relu": hip.relu_bwd_fp8, "sigmoid": hip.sigmoid_bwd_fp8, "tanh": hip.tanh_bwd_fp8}[act](z8, g)
     assert_derivative_codes(codes_of(hip, dz8), values(dz) if dtype == "f32" else None, g64 * SLOPE[act](z64),
                             1e-5 * np.abs(g64), act)
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "tanh"])
+@pytest.mark.parametrize("other", [100.0, -100.0, np.inf, -np.inf, np.nan])
+def test_a_row_does_not_depend_on_the_others(hip, act, other):
+    # 2^25 values of every magnitude, each fourth row's neighbours put past the clip: any dependence on the way
+    # that the others take (an ulp apart in f32) would flip the code of some value near a tie
+    rows, cols = 1 << 16, 512
+    rng = rng_of("neighbours", act)
+    z = (rng.uniform(-20, 20, (rows, 1)) + rng.uniform(-1, 1, (rows, cols))).astype(np.float32)
+    fn = {"sigmoid": hip.sigmoid_fp8, "tanh": hip.tanh_fp8}[act]
+    before = fn(hip.from_numpy(z))
+    z[3::4, 5] = other
+    after = fn(hip.from_numpy(z))
+    keep = np.arange(rows) % 4 != 3
+    for a, b in zip(before, after):
+        assert np.array_equal(a.codes.numpy()[keep], b.codes.numpy()[keep])
+        assert np.array_equal(a.scales.numpy()[:, keep], b.scales.numpy()[:, keep])
+
+
+def test_sigmoid_of_large_negative_arguments(hip):
+    # blocks of e^z down to f32's subnormals, at their own scales (2^-126 at the least)
+    z = np.repeat(np.linspace(-60.0, -115.0, 56), 128).reshape(56, 128).astype(np.float32)
+    z += np.linspace(0, 0.5, 128, dtype=np.float32)
+    h8 = hip.sigmoid_fp8(hip.from_numpy(z), save=False)[0]
+    z64 = z.astype(np.float64)
+    want = np.exp(z64) / (1 + np.exp(z64))
+    scales = h8.scales.numpy()[:, :56]
+    s = 2.0 ** (scales.T.astype(np.float64) - 127)
+    # of the exponent -z log2(e), up to 166: its rounding and the constant's, 2^-17 and 166 2^-25, and an ulp of
+    # exp2 and of the reciprocal: 1.5e-5 of the value, and the steps of the subnormals; then half a code's step
+    tol = 1.5e-5 * want + 2.0**-149
+    low, high = (want - tol).max(axis=1), (want + tol).max(axis=1)
+    got = scales[0].astype(int) - 127  # a block of zeros, as e^z below 2^-149 may give, has the scale 1
+    least = np.where(low > 0, ref.exponents(low), -126)
+    assert ((least <= got) & (got <= ref.exponents(high)) | (low <= 0) & (got == 0)).all()
+    step = np.maximum(2.0 ** (np.floor(np.log2(np.maximum(want / s, 2.0**-6))) - 3), 2.0**-9)
+    assert (np.abs(held(h8) - want) <= step * s / 2 * (1 + 1e-6) + tol).all()
