@@ -35,9 +35,9 @@ constexpr int64_t kNtStoreBytes = 128ll << 20;
 // At least half a round of 256 x 256 tiles: the ping-pong kernel.
 template <bool NT>
 bool launch_pingpong(const Operands& o, uint16_t* c) {
-    const int tiles_m = (o.M + 255) / 256, tiles_n = (o.N + 255) / 256;
+    const int tiles_m = ch::tiles_of(o.M, 256), tiles_n = ch::tiles_of(o.N, 256);
     const int64_t tiles = (int64_t)tiles_m * tiles_n;
-    if (tiles * 2 < ch::num_cus() || tiles > ch::kMaxBlocks / 2) return false;
+    if (tiles * 2 < ch::num_cus() || tiles > INT32_MAX / 2) return false;
     // one workgroup per CU (its LDS); a multiple of 8 keeps a workgroup's tiles on one XCD
     const int64_t resident = ch::num_cus() / 8 * 8;
     const int nt_c = (int64_t)o.M * o.N * 2 >= kNtStoreBytes && o.N % 64 == 0 && ((uintptr_t)c & 127) == 0;
@@ -53,19 +53,25 @@ bool launch_pingpong(const Operands& o, uint16_t* c) {
 }
 
 template <bool NT, bool WIDE, class T, int BM, int BN, int TM, int S>
-void launch_tiled(const Operands& o, T* c, int slices = 1, int64_t part = 0) {
+int32_t launch_tiled(const char* fn, const Operands& o, T* c, int slices = 1, int64_t part = 0) {
     using P = Tiled<BM, BN, TM, S>;
-    const int tiles_m = (o.M + BM - 1) / BM, tiles_n = (o.N + BN - 1) / BN;
-    const unsigned grid = (unsigned)((int64_t)tiles_m * tiles_n * slices);
+    const int tiles_m = ch::tiles_of(o.M, BM), tiles_n = ch::tiles_of(o.N, BN);
+    const int64_t blocks = (int64_t)tiles_m * tiles_n * slices;
+    static_assert(P::THREADS <= 256, "what kMaxBlocks counts");
+    CH_REQUIRE(blocks <= ch::kMaxBlocks, "%s: %d x %d is more than one launch covers", fn, o.M, o.N);
+    const unsigned grid = (unsigned)blocks;
     if constexpr (!NT) {
         if (o.K % P::BK) {
             gemm_fp8_tiled_kernel<false, true, WIDE, T, BM, BN, TM, S>
                 <<<grid, P::THREADS, 0, ch::stream()>>>(o, c, tiles_m, tiles_n, slices, part);
-            return;
+            CH_LAUNCHED(fn);
+            return CLEAVE_HIP_OK;
         }
     }
     gemm_fp8_tiled_kernel<NT, false, WIDE, T, BM, BN, TM, S>
         <<<grid, P::THREADS, 0, ch::stream()>>>(o, c, tiles_m, tiles_n, slices, part);
+    CH_LAUNCHED(fn);
+    return CLEAVE_HIP_OK;
 }
 
 // c[i] = the slices' f32 sums of element i, added in order.
@@ -88,41 +94,28 @@ int32_t launch_layout(const char* fn, const Operands& o, T* c) {
         }
     }
     constexpr bool WIDE = sizeof(T) == 4;
-    auto tiles = [&](int bm, int bn) { return (int64_t)((o.M + bm - 1) / bm) * ((o.N + bn - 1) / bn); };
+    auto tiles = [&](int bm, int bn) { return (int64_t)ch::tiles_of(o.M, bm) * ch::tiles_of(o.N, bn); };
     const int64_t cus = ch::num_cus();
     // Two rounds of 256 x 128 tiles, and they read half the operand bytes of 128 x
     // 128 (us, f32 results: 4096^3 120 against 128, 8192^2 x 1024 151 and 163);
     // below, the smaller tiles lose less to a part-filled round (3000 x 4000 x 2000
     // 56 against 53, 2900^2 x 1000 34 and 32, bf16 2000^2 x 3000 34 and 23).
-    if (tiles(256, 128) >= 2 * cus) {
-        launch_tiled<NT, WIDE, T, 256, 128, 128, 3>(o, c);
-        CH_LAUNCHED(fn);
-        return CLEAVE_HIP_OK;
-    }
+    if (tiles(256, 128) >= 2 * cus) return launch_tiled<NT, WIDE, T, 256, 128, 128, 3>(fn, o, c);
     // Half a round of 128 x 128 tiles, or 64 x 64 (128 against 64, us: 2048^3 f32 24
     // and 31, 1500^3 bf16 15 and 17; below, 512^2 x 4096 21 and 14, 64 x 4096^2 20
     // and 12, 1000^3 11.4 and 9.8).
-    if (tiles(128, 128) * 2 >= cus) {
-        launch_tiled<NT, WIDE, T, 128, 128, 64, 4>(o, c);
-        CH_LAUNCHED(fn);
-        return CLEAVE_HIP_OK;
-    }
+    if (tiles(128, 128) * 2 >= cus) return launch_tiled<NT, WIDE, T, 128, 128, 64, 4>(fn, o, c);
     // Tiles that leave CUs without one: K in slices of at least 8 blocks, less than
     // which the second launch outweighs (whole against sliced, us: 300 x 500 x 16384
     // 36 and 17, 128^2 x 16384 f32 67 and 15, 33 x 4096^2 f32 21 and 13, 512^2 x 4096
     // 13.6 and 12; two slices of 4 blocks, 1000^3: 9.8 and 14).
     const int64_t count = tiles(64, 64), nkb = pitch_of(o.K) / kBlock;
     const int64_t slices = std::min(cus / count, nkb / 8);
-    if (slices <= 1) {
-        launch_tiled<NT, WIDE, T, 64, 64, 32, 6>(o, c);
-        CH_LAUNCHED(fn);
-        return CLEAVE_HIP_OK;
-    }
+    if (slices <= 1) return launch_tiled<NT, WIDE, T, 64, 64, 32, 6>(fn, o, c);
     const int64_t n = (int64_t)o.M * o.N;
     float* const part = (float*)ch::scratch(kPartSlot, sizeof(float) * (size_t)(n * slices));
     if (!part) return CLEAVE_HIP_ERR_OOM;
-    launch_tiled<NT, WIDE, float, 64, 64, 32, 6>(o, part, (int)slices, n);
-    CH_LAUNCHED(fn);
+    CH_OK((launch_tiled<NT, WIDE, float, 64, 64, 32, 6>(fn, o, part, (int)slices, n)));
     sum_parts_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 16 * cus), 256, 0, ch::stream()>>>(
         part, c, n, (int)slices, n);
     CH_LAUNCHED(fn);
@@ -168,8 +161,6 @@ int32_t launch(const char* fn, const Operands& o, T* c, bool nt) {
         const RowsIn<uint8_t> in{nullptr, nullptr, nullptr};
         return nt ? launch_rows<true>(fn, in, o, c) : launch_rows<false>(fn, in, o, c);
     }
-    const int64_t tiles = (int64_t)((o.M + 63) / 64) * ((o.N + 63) / 64);
-    CH_REQUIRE(tiles <= ch::kMaxBlocks, "%s: %d x %d is more than one launch covers", fn, o.M, o.N);
     return nt ? launch_layout<true, T>(fn, o, c) : launch_layout<false, T>(fn, o, c);
 }
 
@@ -342,6 +333,8 @@ int32_t cleave_hip_weight_grad_fp8(const uint8_t* xq, int64_t xqlen, const uint8
                                    int32_t H) {
     const char* fn = "cleave_hip_weight_grad_fp8";
     CH_REQUIRE(B > 0 && D > 0 && H > 0, "%s: B, D and H must be positive (%d, %d, %d)", fn, B, D, H);
+    // the ends of up to 64 slices of whole k-tiles, and the k-tile after one, are ints
+    CH_REQUIRE(B <= INT32_MAX - 4095, "%s: more than %d rows (%d)", fn, INT32_MAX - 4095, B);
     CH_REQUIRE(D <= kMaxPitch && H <= kMaxPitch, "%s: rows of more than %d elements (%d, %d)", fn, kMaxPitch, D, H);
     CH_HELD(fn, xq, xqlen, xs, xslen, B, D);
     CH_REQUIRE(glen == (int64_t)B * H, "%s: glen %lld != B*H (%d x %d)", fn, (long long)glen, B, H);

@@ -39,6 +39,7 @@
 // not stored; a k-row past K reads the last one, which meets A's zero codes.
 #pragma once
 
+#include "extents.hpp"
 #include "fp8.hpp"
 #include "gemm_common.hpp"
 #include "gemm_tiles.hpp"

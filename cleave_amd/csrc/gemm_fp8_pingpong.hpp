@@ -77,7 +77,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_pingpong_kernel(Operands o, uint
         a0 = reinterpret_cast<const char*>(o.a) + m0 * o.pa;
         b0 = reinterpret_cast<const char*>(o.b) + (NT ? n0 * o.pb : n0);
         const bool was_inside = inside;
-        inside = m0 + P::BM <= o.M && (NT ? n0 + P::BN <= o.N : n0 + P::BN <= o.pb);
+        inside = ch::whole_tile(m0, P::BM, o.M) && (NT ? n0 + P::BN <= o.N : n0 + P::BN <= o.pb);
         if (inside && was_inside) return;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {  // 8 rows an instruction: unit rows 0-63 are group 0's, 64-127 group 1's
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(512) void gemm_fp8_pingpong_kernel(Operands o, uint
         first = 0;
         count = min(nkb, P::SEGMENT);
         const int r0 = m0 + grp * P::TM, c0 = n0 + wn * P::TN;
-        const bool whole = m0 + P::BM <= o.M && n0 + P::BN <= o.N;
+        const bool whole = ch::whole_tile(m0, P::BM, o.M) && n0 + P::BN <= o.N;
         tile += (int)gridDim.x;
         const bool more = tile < total;
         if (more) {

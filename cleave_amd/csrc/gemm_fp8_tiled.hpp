@@ -286,7 +286,7 @@ __global__ __launch_bounds__(BM / TM * BN, 2) void gemm_fp8_tiled_kernel(Operand
     // the copies past the last k-tile must land before the LDS is released
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-    if (m0 + BM <= o.M && n0 + BN <= o.N) store_blocks<FM, true>(C, o.M, o.N, m0 + wm, n0 + wn, acc, lane);
+    if (ch::whole_tile(m0, BM, o.M) && n0 + BN <= o.N) store_blocks<FM, true>(C, o.M, o.N, m0 + wm, n0 + wn, acc, lane);
     else store_blocks<FM, false>(C, o.M, o.N, m0 + wm, n0 + wn, acc, lane);
 }
 

@@ -450,7 +450,9 @@ CLEAVE_HIP_API int32_t cleave_hip_index_bwd_f64(double g, double* dt, int64_t le
  * Codes and scales are 16-byte aligned for the products (weight_grad's scales
  * may lie anywhere); the maps need 8 bytes for codes, none for scales.  Outputs
  * may not overlap inputs, except dz = g.  A matrix of no elements is a no-op for
- * the maps and refused by the products. */
+ * the maps and refused by the products.  The row-wise maps (and linear, which
+ * quantises) refuse more than 2^28 - 16 rows of up to 512 columns, half as many of
+ * up to 1024, and so on: what one launch covers. */
 CLEAVE_HIP_API int64_t cleave_hip_fp8_codes_len(int32_t rows, int32_t cols);
 CLEAVE_HIP_API int64_t cleave_hip_fp8_scales_len(int32_t rows, int32_t cols);
 CLEAVE_HIP_API int32_t cleave_hip_quantize_fp8_f32(const float* x, int64_t xlen, uint8_t* q, int64_t qlen, uint8_t* s,
@@ -508,7 +510,7 @@ CLEAVE_HIP_API int32_t cleave_hip_linear_fp8_bf16_bf16(const uint16_t* x, int64_
                                                        int32_t trans_b);
 /* The weight gradient from a layer's saved input: dw[D x H] = x^T g, x [B x D]
  * the values held, g [B x H] in bf16, summed in f32 (the A^T B half of the
- * product rule, stdlib/linalg/matrix.cleave:24). */
+ * product rule, stdlib/linalg/matrix.cleave:24).  At most 2^31 - 4096 rows. */
 CLEAVE_HIP_API int32_t cleave_hip_weight_grad_fp8(const uint8_t* xq, int64_t xqlen, const uint8_t* xs, int64_t xslen,
                                                   const uint16_t* g, int64_t glen, float* dw, int64_t dwlen, int32_t B,
                                                   int32_t D, int32_t H);
