@@ -60,6 +60,8 @@ def answer(w8, rows: np.ndarray) -> np.ndarray:
 
 
 def main(rows: int = 4096, steps: int = 200, lr: float = 0.05) -> dict:
+    if rows < 1 or steps < 1:
+        raise ValueError(f"at least one row and one step, not {rows} and {steps}")
     rng = np.random.default_rng(7)
     x = rng.standard_normal((rows, LAYERS[0]), np.float32)
     shape = list(zip(LAYERS[:-1], LAYERS[1:]))
@@ -69,7 +71,7 @@ def main(rows: int = 4096, steps: int = 200, lr: float = 0.05) -> dict:
     f32, _ = train(forward_f32, x, y, weights, steps, lr)
     fp8, w = train(forward_fp8, x, y, weights, steps, lr)
     w8 = held(w)
-    answers = np.concatenate([answer(w8, x[i:i + 1]) for i in range(8)])
+    answers = np.concatenate([answer(w8, x[i:i + 1]) for i in range(min(8, rows))])
     return {"loss_f32": f32, "loss_fp8": fp8, "served_error": float(np.abs(answers - y[:8]).mean()),
             "answers": answers, "weights": w, "x": x}
 
