@@ -196,9 +196,9 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* p) {
 // Workgroup: 16 rows x U blocks; 16 lanes take a row's block, lane l the
 // columns 8l .. 8l+7 of it.  Sixteen rows make one whole run of scale bytes,
 // the padded rows among them.  f(row, c0, n, kb): columns c0 .. of `row`, n of
-// them inside the matrix (it may be <= 0), or row >= rows.
+// them inside the matrix (it may be <= 0); the row may lie past the last.
 template <int U, class F>
-__device__ __forceinline__ void for_blocks(int rows, int cols, F&& f) {
+__device__ __forceinline__ void for_blocks(int cols, F&& f) {
     const int nb = (int)(pitch_of(cols) / kBlock), nu = (nb + U - 1) / U;
     const int strip = (int)(blockIdx.x / (unsigned)nu), first = (int)(blockIdx.x % (unsigned)nu) * U;
     const int row = strip * kRows + (int)(threadIdx.x >> 4), c = (int)(threadIdx.x & 15) * 8;
@@ -207,7 +207,6 @@ __device__ __forceinline__ void for_blocks(int rows, int cols, F&& f) {
         const int kb = first + i;
         if (kb < nb) f(i, row, kb * kBlock + c, kb);
     }
-    (void)rows;
 }
 
 template <class T, class W>
@@ -215,10 +214,10 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T* __rest
                                                                  uint8_t* __restrict__ s, int rows, int cols) {
     const int64_t pitch = pitch_of(cols), sp = scale_pitch(rows);
     float v[W::U][8];
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int) {
         load8<W::S>(x + (int64_t)row * cols + c, row < rows ? cols - c : 0, v[i]);
     });
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int kb) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int kb) {
         int sb;
         const uint2 w = quantize16(v[i], sb);
         if (row < rows) *reinterpret_cast<uint2*>(q + row * pitch + c) = w;
@@ -291,11 +290,11 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t* __r
     const int64_t pitch = pitch_of(cols), sp = scale_pitch(rows);
     uint2 w[W::U];
     int sb[W::U];
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int kb) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int kb) {
         w[i] = row < rows ? *reinterpret_cast<const uint2*>(q + row * pitch + c) : make_uint2(0, 0);
         sb[i] = s[kb * sp + row];
     });
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int) {
         float v[8];
         decode8(w[i], scale_value(sb[i]), v);
         if (row < rows) store8(out + (int64_t)row * cols + c, cols - c, v);
@@ -309,10 +308,10 @@ __global__ __launch_bounds__(kThreads) void act_kernel(const T* __restrict__ z, 
                                                        uint8_t* __restrict__ zs, int rows, int cols) {
     const int64_t pitch = pitch_of(cols), sp = scale_pitch(rows);
     float v[W::U][8];
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int) {
         load8<W::S>(z + (int64_t)row * cols + c, row < rows ? cols - c : 0, v[i]);
     });
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int kb) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int kb) {
         const int n = row < rows ? cols - c : 0;
         float h[8];
         // One way for the whole wave; an infinity (or a signalling NaN) is past any bound.
@@ -355,12 +354,12 @@ __global__ __launch_bounds__(kThreads) void act_bwd_kernel(const uint8_t* __rest
     float v[W::U][8];
     uint2 w[W::U];
     int sb[W::U];
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int kb) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int kb) {
         w[i] = row < rows ? load_codes<W::S>(zq + row * pitch + c) : make_uint2(0, 0);
         sb[i] = zs[kb * sp + row];
         load8<W::S>(g + (int64_t)row * cols + c, row < rows ? cols - c : 0, v[i]);
     });
-    for_blocks<W::U>(rows, cols, [&](int i, int row, int c, int kb) {
+    for_blocks<W::U>(cols, [&](int i, int row, int c, int kb) {
         float z[8];
         decode8(w[i], scale_value(sb[i]), z);
 #pragma unroll
@@ -395,16 +394,20 @@ bool whole_lines(const T* p, int cols) {
 // wider.  `lines`: the wide matrices are whole 128-byte lines and streamed (bf16
 // 65536 x 4096, sigmoid and its backward, 198 -> 193 and 287 -> 276 us, 8192 x 4096
 // backward 45 -> 37; without whole lines it costs: f32 30000 x 1000, 38 -> 42).
-template <class Go>
+template <bool STREAM = true, class Go>
 int32_t by_blocks(const char* fn, int rows, int cols, bool lines, Go go) {
     const int64_t strips = scale_pitch(rows) / kRows, nb = pitch_of(cols) / kBlock;
     const int64_t wide = strips * ((nb + 3) / 4);
     const bool four = wide >= 4 * (int64_t)ch::num_cus();
     const int64_t blocks = four ? wide : strips * nb;
     CH_REQUIRE(blocks <= ch::kMaxBlocks, "%s: %d x %d is more than one launch covers", fn, rows, cols);
-    if (four && lines) go(Walk<4, true>{}, (unsigned)blocks);
-    else if (four) go(Walk<4, false>{}, (unsigned)blocks);
-    else go(Walk<1, false>{}, (unsigned)blocks);
+    if (!four) {
+        go(Walk<1, false>{}, (unsigned)blocks);
+    } else if (!STREAM || !lines) {
+        go(Walk<4, false>{}, (unsigned)blocks);
+    } else {
+        if constexpr (STREAM) go(Walk<4, true>{}, (unsigned)blocks);
+    }
     CH_LAUNCHED(fn);
     return CLEAVE_HIP_OK;
 }
@@ -552,7 +555,7 @@ template int32_t quantize_fp8<uint16_t>(const char*, const uint16_t*, uint8_t*, 
 template <class T>
 int32_t dequantize_fp8(const char* fn, const uint8_t* q, const uint8_t* s, T* out, int rows, int cols) {
     // what it writes is read next
-    return by_blocks(fn, rows, cols, false, [&](auto walk, unsigned grid) {
+    return by_blocks<false>(fn, rows, cols, false, [&](auto walk, unsigned grid) {
         dequantize_kernel<T, decltype(walk)><<<grid, kThreads, 0, stream()>>>(q, s, out, rows, cols);
     });
 }

@@ -96,11 +96,13 @@ int32_t launch_layout(const char* fn, const Operands& o, T* c) {
     constexpr bool WIDE = sizeof(T) == 4;
     auto tiles = [&](int bm, int bn) { return (int64_t)ch::tiles_of(o.M, bm) * ch::tiles_of(o.N, bn); };
     const int64_t cus = ch::num_cus();
-    // Two rounds of 256 x 128 tiles, and they read half the operand bytes of 128 x
-    // 128 (us, f32 results: 4096^3 120 against 128, 8192^2 x 1024 151 and 163);
-    // below, the smaller tiles lose less to a part-filled round (3000 x 4000 x 2000
-    // 56 against 53, 2900^2 x 1000 34 and 32, bf16 2000^2 x 3000 34 and 23).
-    if (tiles(256, 128) >= 2 * cus) return launch_tiled<NT, WIDE, T, 256, 128, 128, 3>(fn, o, c);
+    // Two rounds of 256 x 128 tiles, f32 results (so many of bf16 are the ping-pong
+    // kernel's): they read half the operand bytes of 128 x 128 (us: 4096^3 120 against
+    // 128, 8192^2 x 1024 151 and 163); below, the smaller tiles lose less to a
+    // part-filled round (3000 x 4000 x 2000 56 against 53, 2900^2 x 1000 34 and 32).
+    if constexpr (WIDE) {
+        if (tiles(256, 128) >= 2 * cus) return launch_tiled<NT, WIDE, T, 256, 128, 128, 3>(fn, o, c);
+    }
     // Half a round of 128 x 128 tiles, or 64 x 64 (128 against 64, us: 2048^3 f32 24
     // and 31, 1500^3 bf16 15 and 17; below, 512^2 x 4096 21 and 14, 64 x 4096^2 20
     // and 12, 1000^3 11.4 and 9.8).
@@ -270,7 +272,7 @@ int32_t weight_grad(const char* fn, const uint8_t* xq, const uint8_t* xs, const 
     // Rows of g of fewer than 4 values: the kernel's chunks of 8 would reach past g's
     // end from more rows than its last one.
     if (wide || H < 4 || ((uintptr_t)dw & 15) != 0) return weight_grad_wide(fn, xq, xs, g, dw, B, D, H);
-    using P = Grad<128>;
+    using P = Grad;
     const int tiles_m = (D + P::BM - 1) / P::BM, tiles_n = (H + P::BN - 1) / P::BN;
     const int64_t tiles = (int64_t)tiles_m * tiles_n, n = (int64_t)D * H, stride = (n + 3) / 4 * 4;
     CH_REQUIRE(tiles <= ch::kMaxBlocks, "%s: %d x %d is more than one launch covers", fn, D, H);
@@ -296,7 +298,7 @@ int32_t weight_grad(const char* fn, const uint8_t* xq, const uint8_t* xs, const 
         slices = 1;
         rows = B;
     }
-    gemm_fp8_grad_kernel<128><<<(unsigned)(tiles * slices), P::GROUPS * P::THREADS, 0, ch::stream()>>>(
+    gemm_fp8_grad_kernel<<<(unsigned)(tiles * slices), P::GROUPS * P::THREADS, 0, ch::stream()>>>(
         xq, xs, g, to, B, D, H, tiles_m, tiles_n, (int)slices, rows, stride);
     CH_LAUNCHED(fn);
     return slices > 1 ? ch::sum_slices_f32(to, dw, n, (int)slices, stride) : CLEAVE_HIP_OK;

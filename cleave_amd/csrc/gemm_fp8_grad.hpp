@@ -7,7 +7,7 @@
 // scale (exact) on its way into LDS, once per tile, and the product is
 // v_mfma_f32_32x32x16_bf16's, f32 sums at the bf16 rate.
 //
-// Tiles of BM x 128 of dw, k-tiles of 32 rows; two groups of four waves, each
+// Tiles of 128 x 128 of dw, k-tiles of 32 rows; two groups of four waves, each
 // with two LDS stages and half of the workgroup's k-tiles, whose sums meet in LDS:
 // two waves a SIMD, and half the slices' sums of two workgroups on a CU.  A k-tile
 // is multiplied from registers while the next one's operands are read and the one
@@ -35,12 +35,11 @@
 namespace ch {
 namespace fp8 {
 
-template <int BM_>
 struct Grad {
-    static constexpr int BM = BM_, BN = 128, BK = 32, NW = 4, GROUPS = 2;
+    static constexpr int BM = 128, BN = 128, BK = 32, NW = 4, GROUPS = 2;
     static constexpr int THREADS = 64 * NW;  // of a group
     static constexpr int WM = BM / 64, WN = NW / WM, TN = BN / WN, FM = 2, FN = TN / 32;  // waves of 64 x TN
-    static constexpr int A_BYTES = BK * 256, B_BYTES = BK * BN * 2, STAGE = A_BYTES + B_BYTES;
+    static constexpr int A_BYTES = BK * BM * 2, B_BYTES = BK * BN * 2, STAGE = A_BYTES + B_BYTES;
     static constexpr int PF = 4;  // k-tiles whose loads are in flight, in registers
     static constexpr int CHUNKS_A = BK * BM / 16 / THREADS;  // of 16 codes a thread
     static constexpr int CHUNKS_B = BK * BN / 8 / THREADS;   // of 8 values
@@ -51,15 +50,12 @@ struct Grad {
 typedef float v4f __attribute__((ext_vector_type(4)));
 struct __attribute__((packed)) PackedChunk { v4u v; };
 
-template <int BM>
-__global__ __launch_bounds__(512, 2) void gemm_fp8_grad_kernel(const uint8_t* __restrict__ xq,
-                                                               const uint8_t* __restrict__ xs,
-                                                               const uint16_t* __restrict__ g, float* __restrict__ dw,
-                                                               int B, int D, int H, int tiles_m, int tiles_n, int slices,
-                                                               int rows_per_slice, int64_t slice_stride) {
-    using P = Grad<BM>;
-    constexpr int BN = P::BN, BK = P::BK, FM = P::FM, FN = P::FN, PF = P::PF;
-    // A keeps 256-byte rows whatever BM: the swizzle's banks
+static __global__ __launch_bounds__(512, 2) void gemm_fp8_grad_kernel(
+    const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xs, const uint16_t* __restrict__ g,
+    float* __restrict__ dw, int B, int D, int H, int tiles_m, int tiles_n, int slices, int rows_per_slice,
+    int64_t slice_stride) {
+    using P = Grad;
+    constexpr int BM = P::BM, BN = P::BN, BK = P::BK, FM = P::FM, FN = P::FN, PF = P::PF;
     __shared__ __attribute__((aligned(1024))) char lds[P::GROUPS][2][P::STAGE];
     const int lane = threadIdx.x & 63, tid = (int)threadIdx.x % P::THREADS;
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / P::THREADS);

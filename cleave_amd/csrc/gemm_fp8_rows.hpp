@@ -30,7 +30,6 @@ namespace fp8 {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-
 // Where a lane's 8 values of matrix instruction t lie in a k-block.
 template <bool NT>
 __device__ __forceinline__ int k_of(int g, int t) {
