@@ -146,11 +146,13 @@ struct Sigmoid {
     static __device__ __forceinline__ float fwd(float z) {
         return z < -kNear ? exp2_down(kLog2e * z) : fwd_near(z);
     }
-    // in u = e^-|z|, which neither overflows nor cancels for a large |z|
+    // q (1 - q), q = 1 - s of |z| = u / (1 + u) in u = e^-|z|: nothing overflows or
+    // cancels for a large |z|, and as q - q q it is at most 1/4 however q is rounded
+    // (u r r passed it, and the scale of a block whose largest g is 1.75 2^k with it).
     static __device__ __forceinline__ float bwd(float z, float g) {
         const float u = __builtin_amdgcn_exp2f(-kLog2e * __builtin_fabsf(z));
-        const float r = __builtin_amdgcn_rcpf(1.0f + u);
-        return g * (u * r * r);
+        const float q = u * __builtin_amdgcn_rcpf(1.0f + u);
+        return g * __builtin_fmaf(-q, q, q);
     }
 };
 struct Tanh {
@@ -163,10 +165,11 @@ struct Tanh {
         const float near = a * (1.0f + w * (-1.0f / 3.0f + w * (2.0f / 15.0f - w * (17.0f / 315.0f))));
         return __builtin_copysignf(a < 0.125f ? near : far, z);
     }
+    // 4 q (1 - q), q = (1 - tanh |z|) / 2 = u / (1 + u): at most 1, as above
     static __device__ __forceinline__ float bwd(float z, float g) {
         const float u = __builtin_amdgcn_exp2f(-2.0f * kLog2e * __builtin_fabsf(z));
-        const float r = __builtin_amdgcn_rcpf(1.0f + u);
-        return g * (4.0f * u * r * r);
+        const float q = u * __builtin_amdgcn_rcpf(1.0f + u);
+        return g * (4.0f * __builtin_fmaf(-q, q, q));
     }
 };
 

@@ -206,3 +206,24 @@ def test_sigmoid_of_large_negative_arguments(hip):
     assert ((least <= got) & (got <= ref.exponents(high)) | (low <= 0) & (got == 0)).all()
     step = np.maximum(2.0 ** (np.floor(np.log2(np.maximum(want / s, 2.0**-6))) - 3), 2.0**-9)
     assert (np.abs(held(h8) - want) <= step * s / 2 * (1 + 1e-6) + tol).all()
+
+
+@pytest.mark.parametrize("act,top", [("sigmoid", 0.25), ("tanh", 1.0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_derivative_is_at_most_its_largest(hip, act, top, dtype):
+    # z near 0, where the slope is its largest but for less than f32 holds: every code at scales down to 2^-40.
+    # g = 1.75 puts the largest dz of each block (z = 0) on the edge between two scales: an ulp more doubles it.
+    codes = np.zeros((40, 256), np.uint8)
+    codes[:, :127], codes[:, 128:255] = np.arange(127), 128 + np.arange(127)
+    scales = np.full((2, 48), 127, np.uint8)
+    scales[:, :40] = 127 - 8 - np.arange(40)  # |z| up to 1.75 2^0, 2^-1, ...
+    z8 = hip.empty_fp8((40, 256))
+    z8.codes.upload(codes)
+    z8.scales.upload(scales)
+    g = np.full((40, 256), 1.75, np.float32)
+    dz, dz8 = {"sigmoid": hip.sigmoid_bwd_fp8, "tanh": hip.tanh_bwd_fp8}[act](
+        z8, hip.from_numpy(g if dtype == "f32" else ref.to_bf16(g), dtype))
+    assert (values(dz) <= 1.75 * top).all()
+    assert (dz8.scales.numpy()[:, :40].astype(int) - 127 == ref.exponents(np.array(1.75 * top))).all()
+    z64 = held(z8)
+    assert (np.abs(held(dz8) - 1.75 * SLOPE[act](z64)) <= 1.75 * top / 16 + 1e-5).all()
