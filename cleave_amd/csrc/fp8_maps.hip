@@ -7,7 +7,9 @@
 // when the scale is known.  All of it is bound by HBM bytes: bf16 65536 x 4096
 // sigmoid with its checkpoint 187 us (1.08 GB, 5.8 TB/s), its backward with both
 // results 276 us (1.62 GB, 5.9 TB/s), an f32 8192^2 weight 57 us (0.34 GB, 5.9
-// TB/s); 1000 x 500 is one launch, 3 us of it the kernel.
+// TB/s), each pass on other matrices than the one before; on the same ones again the
+// last-level cache still holds a part (the backward 240 us).  1000 x 500 is one
+// launch, 3 us of it the kernel.
 #include <type_traits>
 
 #include "fp8.hpp"
@@ -395,7 +397,7 @@ bool whole_lines(const T* p, int cols) {
 // go(Walk, grid of for_blocks<Walk::U>).  Four blocks a thread keep eight loads in
 // flight; with fewer workgroups than fill the card, one block each spreads the work
 // wider.  `lines`: the wide matrices are whole 128-byte lines and streamed (bf16
-// 65536 x 4096, sigmoid and its backward, 198 -> 193 and 287 -> 276 us, 8192 x 4096
+// 65536 x 4096, sigmoid and its backward, 189 -> 186 and 287 -> 281 us, 8192 x 4096
 // backward 45 -> 37; without whole lines it costs: f32 30000 x 1000, 38 -> 42).
 template <bool STREAM = true, class Go>
 int32_t by_blocks(const char* fn, int rows, int cols, bool lines, Go go) {

@@ -19,10 +19,11 @@
 // in order by another launch; a slice's tiles run on one XCD, or each of the eight
 // would fetch its rows.
 //
-// What bounds it: the LDS, busy for 670 of the 1390 cycles a CU takes for a k-tile
-// of each group (the matrix instructions for 512), and the way in and out: 2048^3
-// takes 23 us (750 TFLOP/s), of which 9 do not depend on the rows; 10000 x 784 x
-// 500 24 us with its sums (1.6 MB of dw as 13 MB of slices).  Against one group and
+// What bounds it: no unit alone.  The LDS is busy 0.48 of 2048^3's cycles and 0.38 of
+// 10000 x 784 x 500's (0.09 and 0.07 of them for conflicts), the matrix instructions
+// 0.34 and 0.25; the rest is waits of a k-tile's chain and the way in and out: 2048^3
+// takes 23 to 25 us (690-750 TFLOP/s), of which 8 do not depend on the rows (256 rows
+// take 9.9); 10000 x 784 x 500 23 us with its sums (1.6 MB of dw as 13 MB of slices).  Against one group and
 // two workgroups a CU: 2048^3 33 -> 23 us, 4096 x 1024^2 26 -> 24, 65536 x 512^2 47 ->
 // 44, 10000 x 784 x 500 22 -> 24, 100 x 2000 x 1000 7 -> 8.
 #pragma once

@@ -10,21 +10,21 @@
 //
 // A k-block of 128 takes two phases: phase x = 0, 1 multiplies half x of the
 // wave's rows, over the whole k-block, by columns that stay in registers for
-// both.  So a k-contiguous operand is copied in whole 128-byte lines.  Copied in
-// k-tiles of 64 bytes a row, its L2 requests (two for each line) took 72% of
-// what the channels can serve and held the matrix cores to 67% (8192^3 A.B^T 454
-// us).
+// both.  So a k-contiguous operand is copied in whole 128-byte lines (in k-tiles of
+// 64 bytes a row, two L2 requests for each line, 8192^3 A.B^T took 454 us).
 // One workgroup a CU walks its tiles, so that the stores of one overlap the first
 // k-blocks of the next.
 // LDS: four units of A (128 rows x 128 bytes, half x of both groups' rows), two
 // of B (32 KiB), and the scales of 64 k-blocks, 256 + 256 bytes each; K is
 // walked in segments of 8192.
 //
-// What bounds it: power.  In a loop of 8192^3 products the cards' clock falls to
-// 1.25 GHz (1.42 in 65536 x 4096 x 1024, whose C is 512 MiB), at which the
-// matrix cores are busy 94% of a tile's k-blocks: 437 us, 2.5 PFLOP/s; the first
-// product after a pause runs in 370.  Waiting less gave nothing any more there
-// (starts staggered over a tile's time, 334 against 334 us).
+// What bounds it: for 8192^3 the matrix cores, busy 0.90 of the cycles in which the
+// shader engines are, at the clock that power leaves (1.6-1.7 GHz): 376 us (A.B) and
+// 382 (A.B^T) in a loop, 2.9 PFLOP/s.  65536 x 4096 x 1024 keeps them busy 0.56: 8
+// k-blocks between a tile's first copies and its stores, 512 MiB of C in all; 273 us in
+// a loop, 2.0 PFLOP/s.  Waiting less in the loop gave 8192^3 nothing any more.
+// Just past a whole round of tiles the last one is paid in full (4096^2 x 8192 100 us,
+// 4352 x 4096 x 8192, 16 tiles more, 157).
 #pragma once
 
 #include "gemm_fp8_tiled.hpp"
